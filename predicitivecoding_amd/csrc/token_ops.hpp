@@ -186,11 +186,88 @@ struct Teacher {
     float temperature;
 };
 
+// How a loss goes about its call: which kernels, their tiles, and what stays in scratch.
+struct LossPlan {
+    bool grads, few, in_place, last_copy, coded, slim, close;
+    int ob, unit, pitch;                 // bytes of an element, elements of a load, the packed hidden states' row
+    int few_nr, few_blocks, few_across, few_step, few_span, few_ranges, few_y;
+    int stack;                           // rows apart of the two parts of G (0: one part)
+    size_t rows_pad;                     // rows of G and of the packed hidden states
+    long long wld;                       // row pitch of W, or of its copy
+    int v0, buckets, top, t_lse, slots;
+    int width;                           // of the vocabulary's pieces
+    int z_cols;                          // columns whose logits are kept
+    int dh_rows, dh_k, dh_most, dw_ids, t;
+    size_t dh_units;
+};
+LossPlan plan_loss(const TokCall& c, const void* weight, long long ldw, int rows, int dim, int vocab, int top, bool d_hidden,
+                   bool d_weight, size_t keep) {
+    LossPlan p;
+    std::memset(&p, 0, sizeof p);
+    const int ob = p.ob = op_bytes(c.dtype), unit = p.unit = 16 / ob, pitch = p.pitch = (int)round_up(dim, kFeatPad);
+    const int v64 = (int)round_up(vocab, 64);
+    p.grads = d_hidden || d_weight;
+    // A few rows stream W (few_rows_kernel, few_grads_kernel), if the hidden states
+    // fit beside each other in LDS and the limit lets their logits be kept.
+    p.few_nr = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+    p.few = rows <= (ob == 4 ? kFewTok : kFewTok16) && dim >= unit && p.few_nr * pitch * ob <= kFewLds && (size_t)rows * 4 * v64 <= keep;
+    // Up to kTokStackRows rows of a 16-bit type: gradients in two parts (grad_rows_kernel).
+    // Their logits are kept whole, which a low limit forbids.
+    p.stack = !p.few && p.grads && ob == 2 && rows <= kTokStackRows && round_up(rows, 32) * 8 * v64 <= keep ? (int)round_up(rows, 32) : 0;
+    p.rows_pad = p.stack ? 2 * p.stack : round_up(rows, 64);
+    // W is read in place where its rows are whole 32-bit words, which the tiles'
+    // loads take, and what a K sweep reads past a row's end is the next row
+    // (multiplied by zeros); else a padded copy is.
+    p.in_place = whole_words(weight, ldw, ob) && (dim % kFeatPad == 0 || (ldw == dim && dim >= kFeatPad));
+    p.wld = p.in_place ? ldw : pitch;
+    // The last rows' copy: where a sweep would read past the matrix's end.
+    p.v0 = (vocab - 1) / 256 * 256;
+    p.last_copy = p.in_place && !p.few && (dim % kFeatPad != 0 || (d_hidden && vocab % 64 != 0));
+    p.buckets = (vocab + kTokBucket - 1) / kTokBucket;
+    p.top = top;
+
+    p.t_lse = logits_tile(c, rows, vocab, dim);
+    p.few_blocks = std::max(1, std::min(4 * c.cus, (vocab + 15) / 16));
+    // few_grads_kernel: as many workgroups as the CUs hold at once (four of one or two
+    // rows, two of more: calls of 2 x 16832 x 1536 fp32 with four and two a CU 75 / 87 us,
+    // 1 x 32768 x 4096 bf16 169 / 176, 4 x 32768 x 4096 199 / 187), over the columns
+    // first, and shorter turns of the waves rather than fewer.
+    const int few_cols = (dim + 64 * unit - 1) / (64 * unit);
+    p.few_across = std::min(4, few_cols);
+    p.few_y = (few_cols + 3) / 4;
+    const int few_ways = 4 / p.few_across, few_want = ((p.few_nr <= 2 ? 4 : 2) * c.cus + p.few_y - 1) / p.few_y;
+    const int few_ids = vocab / (few_ways * few_want);
+    p.few_step = few_ids >= 64 ? 64 : few_ids >= 32 ? 32 : 16;   // whole parts of a bucket
+    p.few_span = (int)round_up((vocab + few_want - 1) / few_want, few_ways * p.few_step);
+    p.few_ranges = (vocab + p.few_span - 1) / p.few_span;
+    p.slots = p.few ? p.few_blocks : (vocab + p.t_lse - 1) / p.t_lse;
+    // pieces of the vocabulary, of like width
+    p.width = (int)std::max<size_t>(256, std::min<size_t>(round_up(vocab, 256), kTokPieceBytes / (p.rows_pad * ob) / 256 * 256));
+    const int pieces = (vocab + p.width - 1) / p.width;
+    p.width = (int)round_up((vocab + pieces - 1) / pieces, 256);
+    p.coded = c.dtype == PCD_BF16 && !p.few && !p.stack;   // kept logits: 17 bits each, or 32
+    // All columns where they fit the limit (a stacked call's do), else whole pieces.
+    const size_t fit = keep / (p.rows_pad * (p.coded ? 17 : 32) / 8);
+    p.z_cols = p.few || (p.grads && fit >= (size_t)v64) ? v64 : p.grads ? (int)(fit / p.width * p.width) : 0;
+    // Few rows with every logit kept: grad_rows_kernel closes the losses.
+    p.close = p.grads && !p.few && p.z_cols >= vocab && pieces == 1 && p.rows_pad * ((vocab + kGradCols - 1) / kGradCols) <= (size_t)8 * c.cus;
+    // Few rows, all of rows_pad always padded: DW in a kernel of its own (slim_dw_kernel).
+    p.slim = d_weight && !p.few && ob == 2 && (p.stack || p.rows_pad == 64) && dim >= kSlimLeast &&
+             (!d_hidden || (size_t)vocab * dim * ob >= kSlimBytes);
+    p.dh_rows = !d_hidden || p.few ? 0 : p.stack ? (int)p.rows_pad : rows;
+    p.dw_ids = d_weight && !p.slim && !p.few ? std::min(p.width, vocab) : 0;
+    p.dh_k = std::min(p.width, vocab);                                     // K of a piece
+    const int dh_least = vocab - (vocab - 1) / p.width * p.width;   // ... and of the last
+    p.dh_most = std::max(1, std::min(64, dh_least / 128));
+    p.t = pair_tile(c, p.dh_rows, dim, p.dh_k, p.dh_most, p.dw_ids, (int)p.rows_pad);
+    p.dh_units = d_hidden && !p.few ? std::max<size_t>(tile_count(p.dh_rows, dim, p.t), p.dh_most > 1 ? 2 * c.cus : 0) : 0;
+    return p;
+}
+
 // Both losses (`teacher` null: cross entropy).
 int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, const void* weight, long long ldw,
                const int* labels, const Teacher* teacher, const float* row_weight, int rows, int dim, int vocab, float scale,
                float* loss, void* d_hidden, long long ld_dh, void* d_weight, long long ld_dw, hipStream_t s) {
-    const int ob = op_bytes(dtype);
     if (rows == 0) {
         if (!d_weight) return PCD_SUCCESS;
         return with_type(dtype, [&](auto* td) {   // a sum over no rows
@@ -203,56 +280,15 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
     }
     TokCall c{dtype, 0, s, {}};
     if (int st = device_cus(&c.cus)) return st;
-    const bool grads = d_hidden || d_weight;
-    const int pitch = (int)round_up(dim, kFeatPad);
-    const size_t keep = g_keep_logits.load(std::memory_order_relaxed);
-    const int unit = 16 / ob;   // elements of a load
-    // A few rows stream W (few_rows_kernel, few_grads_kernel), if the hidden states
-    // fit beside each other in LDS and the limit lets their logits be kept.
-    const int few_nr = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
-    const bool few = rows <= (ob == 4 ? kFewTok : kFewTok16) && dim >= unit && few_nr * pitch * ob <= kFewLds && (size_t)rows * 4 * round_up(vocab, 64) <= keep;
-    // Up to kTokStackRows rows of a 16-bit type: gradients in two parts (grad_rows_kernel).
-    // Their logits are kept whole, which a limit near none at all forbids.
-    const int stack = !few && grads && ob == 2 && rows <= kTokStackRows && round_up(rows, 32) * 8 * round_up(vocab, 64) <= keep
-                          ? (int)round_up(rows, 32) : 0;
-    const size_t rows_pad = stack ? 2 * stack : round_up(rows, 64);
-    // W is read in place where its rows are whole 32-bit words, which the tiles'
-    // loads take, and what a K sweep reads past a row's end is the next row
-    // (multiplied by zeros); else a padded copy is.
-    const bool in_place = whole_words(weight, ldw, ob) && (dim % kFeatPad == 0 || (ldw == dim && dim >= kFeatPad));
-    const long long wld = in_place ? ldw : pitch;
-    // The last rows' copy: where a sweep would read past the matrix's end.
-    const int v0 = (vocab - 1) / 256 * 256;
-    bool last_copy = in_place && (dim % kFeatPad != 0 || (d_hidden && vocab % 64 != 0));
-    const int buckets = (vocab + kTokBucket - 1) / kTokBucket, top = teacher ? teacher->top : 1;
-
-    const int t_lse = logits_tile(c, rows, vocab, dim);
-    last_copy = last_copy && !few;
-    const int few_blocks = std::max(1, std::min(4 * c.cus, (vocab + 15) / 16));
-    // few_grads_kernel: as many workgroups as the CUs hold at once (four of one or two
-    // rows, two of more: calls of 2 x 16832 x 1536 fp32 with four and two a CU 75 / 87 us,
-    // 1 x 32768 x 4096 bf16 169 / 176, 4 x 32768 x 4096 199 / 187), over the columns
-    // first, and shorter turns of the waves rather than fewer.
-    const int few_cols = (dim + 64 * unit - 1) / (64 * unit), few_across = std::min(4, few_cols), few_y = (few_cols + 3) / 4;
-    const int few_ways = 4 / few_across, few_want = ((few_nr <= 2 ? 4 : 2) * c.cus + few_y - 1) / few_y;
-    const int few_ids = vocab / (few_ways * few_want), few_step = few_ids >= 64 ? 64 : few_ids >= 32 ? 32 : 16;   // whole parts of a bucket
-    const int few_span = (int)round_up((vocab + few_want - 1) / few_want, few_ways * few_step), few_ranges = (vocab + few_span - 1) / few_span;
-    const int slots = few ? few_blocks : (vocab + t_lse - 1) / t_lse;
-    // pieces of the vocabulary, of like width
-    int width = (int)std::max<size_t>(256, std::min<size_t>(round_up(vocab, 256), kTokPieceBytes / (rows_pad * ob) / 256 * 256));
-    const int pieces = (vocab + width - 1) / width;
-    width = (int)round_up((vocab + pieces - 1) / pieces, 256);
-    const bool coded = dtype == PCD_BF16 && !few && !stack;   // kept logits: 17 bits each, or 32
-    const int z_cols = few ? (int)round_up(vocab, 64)
-                       : grads ? (int)std::min<size_t>(round_up(vocab, 64), keep / (rows_pad * (coded ? 17 : 32) / 8) / width * width) : 0;
-    // Few rows, all of rows_pad always padded: DW in a kernel of its own (slim_dw_kernel).
-    const bool slim = d_weight && !few && ob == 2 && (stack || rows_pad == 64) && dim >= kSlimLeast &&
-                      (!d_hidden || (size_t)vocab * dim * ob >= kSlimBytes);
-    const int dh_rows = !d_hidden || few ? 0 : stack ? (int)rows_pad : rows, dw_ids = d_weight && !slim && !few ? std::min(width, vocab) : 0;
-    const int dh_k = std::min(width, vocab), dh_least = vocab - (vocab - 1) / width * width;   // K of a piece, and of the last
-    const int dh_most = std::max(1, std::min(64, dh_least / 128));
-    const int t = pair_tile(c, dh_rows, dim, dh_k, dh_most, dw_ids, (int)rows_pad);
-    const size_t dh_units = d_hidden && !few ? std::max<size_t>(tile_count(dh_rows, dim, t), dh_most > 1 ? 2 * c.cus : 0) : 0;
+    const LossPlan plan = plan_loss(c, weight, ldw, rows, dim, vocab, teacher ? teacher->top : 1, d_hidden, d_weight,
+                                    g_keep_logits.load(std::memory_order_relaxed));
+    const bool grads = plan.grads, few = plan.few, in_place = plan.in_place, last_copy = plan.last_copy, coded = plan.coded;
+    const bool slim = plan.slim, close = plan.close;
+    const int ob = plan.ob, unit = plan.unit, pitch = plan.pitch, stack = plan.stack, v0 = plan.v0, buckets = plan.buckets;
+    const int top = plan.top, slots = plan.slots, width = plan.width, z_cols = plan.z_cols, dh_rows = plan.dh_rows, t = plan.t;
+    const int few_nr = plan.few_nr, few_blocks = plan.few_blocks, few_ranges = plan.few_ranges, few_y = plan.few_y;
+    const size_t rows_pad = plan.rows_pad, dh_units = plan.dh_units;
+    const long long wld = plan.wld;
 
     Arena m;
     const size_t o_ctl = m.add(sizeof(TokCtl)), o_map = m.add((size_t)rows * 4), o_rank = m.add((size_t)rows * 4);
@@ -330,7 +366,7 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
         ra.map = m.at<int>(o_map);
         ra.rank = m.at<int>(o_rank);
         ra.loss = loss;
-        ra.dh = RangeArgs{t, (dim + t - 1) / t, dh_k, tile_ends(t), dh_most, c.cus};
+        ra.dh = RangeArgs{t, (dim + t - 1) / t, plan.dh_k, tile_ends(t), plan.dh_most, c.cus};
         ra.stack = stack;
         ra.clear = (u32x4*)c.split.count;
         ra.clear_units = (int)(count_bytes / 16);
@@ -366,7 +402,7 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
         if (few) k.taken = nullptr;   // its logits are there
         const float alpha = scale * (teacher ? teacher->temperature : 1.f);
         const int nt = (size_t)vocab * dim * ob > kTokPieceBytes;
-        const FewArgs fa{hidden, ldh, dim, vocab, pitch, few_across, few_step, few_span, weight, ldw, d_hidden ? m.at<float>(o_dh) : nullptr,
+        const FewArgs fa{hidden, ldh, dim, vocab, pitch, plan.few_across, plan.few_step, plan.few_span, weight, ldw, d_hidden ? m.at<float>(o_dh) : nullptr,
                          d_weight, ld_dw, alpha, nt};
         const int row_blocks = (int)((stack ? (size_t)stack : rows_pad) / 4);
         const dim3 grid(row_blocks + (last_copy ? 32 : 0), (pitch + kGatherCols - 1) / kGatherCols);
@@ -427,9 +463,7 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
             return logits_product(c, epi, t, p, a, kk);
         };
         if (!few)
-            if (int st = logits(EPI_TOK_LSE, t_lse, 0, vocab, nullptr, 0)) return st;
-        // Few rows with every logit kept: grad_rows_kernel closes the losses.
-        const bool close = grads && !few && z_cols >= vocab && pieces == 1 && rows_pad * ((vocab + kGradCols - 1) / kGradCols) <= (size_t)8 * c.cus;
+            if (int st = logits(EPI_TOK_LSE, plan.t_lse, 0, vocab, nullptr, 0)) return st;
         if (!close && !(few && grads)) {
             hipLaunchKernelGGL(row_loss_kernel, dim3(rows), dim3(256), 0, s, k);
             if (int st = from_hip(hipGetLastError(), "row_loss_kernel launch")) return st;
