@@ -187,7 +187,8 @@ int pcd_gemm_f16_batched(const uint16_t* dA, const uint16_t* dB, float* dC, int 
  * `weight` whose rows are not whole 32-bit words, or are apart and no multiple
  * of 64 wide, into a copy of whole 128-byte rows).  Types are enum pcd_dtype,
  * 16-bit ones as raw bit patterns.  Sums and softmax statistics are fp32.  Where two types are
- * given they are the same or one of them is PCD_F32.  Results do not depend on
+ * given they are the same or one of them is PCD_F32.  A loss takes up to 2^24
+ * rows, ids and 2^39 logits, and a dim of up to 2^20.  Results do not depend on
  * the launch's timing: the same inputs give the same bits.  Scratch comes from
  * the library's pool.  Asynchronous on `stream`. */
 

@@ -341,12 +341,16 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const RowArgs a, const
 
 constexpr int kMaxTop = 1024;
 
+// Row of a workgroup in a grid of one for each row (row_grid; kGridUnits).
+__device__ __forceinline__ int grid_row() { return (int)(blockIdx.y * gridDim.x + blockIdx.x); }
+inline dim3 row_grid(int rows) { return dim3(std::min(rows, kGridUnits), (rows + kGridUnits - 1) / kGridUnits); }
+
 // One row's slots: sorted by id (a slot's place is the number of smaller ids and
 // of equal ones before it), probabilities softmax(t / T) over the slots that
 // are there, those of equal ids summed into the first; where each bucket of 64
 // ids begins; sum p ln p; and whether the row has a slot at all.
 template <typename TT>
-__global__ void __launch_bounds__(256) teacher_kernel(const int* __restrict__ ids, const TT* __restrict__ logits, int top,
+__global__ void __launch_bounds__(256) teacher_kernel(const int* __restrict__ ids, const TT* __restrict__ logits, int rows, int top,
                                                       int vocab, float inv_t, int buckets, int* __restrict__ out_ids,
                                                       float* __restrict__ out_probs, uint16_t* __restrict__ starts,
                                                       float* __restrict__ plogp, int* __restrict__ marks) {
@@ -354,7 +358,8 @@ __global__ void __launch_bounds__(256) teacher_kernel(const int* __restrict__ id
     __shared__ float raw_t[kMaxTop], t[kMaxTop];
     __shared__ float fred[4];
     __shared__ int ired[4];
-    const size_t row = blockIdx.x;
+    const size_t row = grid_row();
+    if (row >= (size_t)rows) return;
     const int none = 0x7FFFFFFF;
     float m = -__builtin_inff();
     int past = 0;
@@ -474,12 +479,12 @@ __device__ __forceinline__ void close_row(const TokArgs& t, int orig, float l2, 
     if (t.labels == nullptr) x.got = block_join(x.got, fred, [](float x, float y) { return x + y; });
     if (threadIdx.x == 0) t.loss[orig] = x.w * t.factor * (x.plogp + 0.6931471805599453f * (l2 - x.got));
 }
-__global__ void __launch_bounds__(256) row_loss_kernel(const TokArgs t) {
+__global__ void __launch_bounds__(256) row_loss_kernel(const TokArgs t, int rows) {
     __shared__ float fred[4];
     __shared__ float2 red[4];
-    const int r = blockIdx.x, live = gld(&t.ctl->live), orig = gld(t.map + r);   // (past the live rows: whatever is there)
+    const int r = min(grid_row(), rows - 1), live = gld(&t.ctl->live), orig = gld(t.map + r);   // (past the live rows: whatever is there)
     const float2 mine = row_share(t, r, threadIdx.x, 256);
-    if (r >= live) return;
+    if (grid_row() >= live) return;
     const RowTarget x = row_target(t, r, orig);
     const float l2 = join_shares(mine, red);
     if (threadIdx.x == 0) t.lse2[r] = l2;

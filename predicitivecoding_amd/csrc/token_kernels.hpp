@@ -100,7 +100,12 @@ struct TokArgs {
     // LSE, GRAD: column tile last_tn reads W's last rows from their copy (null: in place)
     const void* b_last;
     int last_tn;
+    int unit0;                   // LSE, GRAD: the launch's first work unit (see kGridUnits)
 };
+
+// Workgroups of one launch at most: HIP takes fewer than 2^32 threads in a grid,
+// and a workgroup has up to 512.  Whole rounds over the XCDs.
+constexpr int kGridUnits = 1 << 22;
 
 __device__ __forceinline__ int tok_rows(const TokArgs* t, int epi) {
     return __builtin_amdgcn_readfirstlane(
@@ -372,8 +377,8 @@ template <typename OP, int BM, int BN, int EPI>
 __global__ void __launch_bounds__((TileCfg<BM, BN, OpTraits<OP>::bytes>::NT), (TileCfg<BM, BN, OpTraits<OP>::bytes>::OCC))
 tok_kernel(const Problem p, const PhaseArgs args, const TokArgs tok) {
     __shared__ __attribute__((aligned(16))) char smem[phase_smem_bytes<OP, BM, BN>()];
-    phase_unit<OP, BM, BN, EPI>((KProblem*)__builtin_amdgcn_kernarg_segment_ptr(), 1, args, blockIdx.x, gridDim.x, smem,
-                                &tok);
+    phase_unit<OP, BM, BN, EPI>((KProblem*)__builtin_amdgcn_kernarg_segment_ptr(), 1, args, tok.unit0 + blockIdx.x, gridDim.x,
+                                smem, &tok);
 }
 
 // DH on the first dh_grid workgroups and DW on the rest (either may have none).

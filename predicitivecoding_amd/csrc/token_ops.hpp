@@ -147,7 +147,13 @@ int grid_of(size_t units) { return (int)((units + kXcds - 1) / kXcds * kXcds); }
 int logits_product(const TokCall& c, int epi, int t, Problem p, PhaseArgs a, const TokArgs& k) {
     lay_tiles(c, t, p, a, true);
     return with_type(c.dtype, [&](auto* op) {
-        return launch_token_op<std::remove_pointer_t<decltype(op)>>(t, epi, p, a, k, grid_of(p.tiles), c.s);
+        const int grid = grid_of(p.tiles);
+        TokArgs kk = k;
+        for (kk.unit0 = 0; kk.unit0 < grid; kk.unit0 += kGridUnits) {
+            const int st = launch_token_op<std::remove_pointer_t<decltype(op)>>(t, epi, p, a, kk, std::min(grid - kk.unit0, kGridUnits), c.s);
+            if (st) return st;
+        }
+        return (int)PCD_SUCCESS;
     });
 }
 
@@ -347,8 +353,8 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
             k.factor = teacher->temperature * teacher->temperature;
             with_type(teacher->dtype, [&](auto* tt) {
                 using TT = std::remove_pointer_t<decltype(tt)>;
-                hipLaunchKernelGGL(teacher_kernel<TT>, dim3(rows), dim3(256), 0, s, teacher->ids, (const TT*)teacher->logits,
-                                   top, vocab, inv_t, buckets, m.at<int>(o_ids), m.at<float>(o_probs),
+                hipLaunchKernelGGL(teacher_kernel<TT>, row_grid(rows), dim3(256), 0, s, teacher->ids, (const TT*)teacher->logits,
+                                   rows, top, vocab, inv_t, buckets, m.at<int>(o_ids), m.at<float>(o_probs),
                                    m.at<uint16_t>(o_starts), m.at<float>(o_plogp), m.at<int>(o_marks));
                 return 0;
             });
@@ -465,7 +471,7 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
         if (!few)
             if (int st = logits(EPI_TOK_LSE, plan.t_lse, 0, vocab, nullptr, 0)) return st;
         if (!close && !(few && grads)) {
-            hipLaunchKernelGGL(row_loss_kernel, dim3(rows), dim3(256), 0, s, k);
+            hipLaunchKernelGGL(row_loss_kernel, row_grid(rows), dim3(256), 0, s, k, rows);
             if (int st = from_hip(hipGetLastError(), "row_loss_kernel launch")) return st;
         }
         if (!grads) return PCD_SUCCESS;
@@ -576,6 +582,9 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
     return st ? st : st2;
 }
 
+// Most logits of a call: 2^27 tiles of 64 x 64, which the deal of tiles over the XCDs counts in eighths of an int.
+constexpr long long kMostLogits = 1ll << 39;
+
 // The checks both losses make.
 int check_loss(const char* name, int dtype, const void* hidden, int hidden_dtype, long long* ldh, const void* weight,
                long long* ldw, int rows, int dim, int vocab, float scale, const float* loss, long long* ld_dh,
@@ -586,6 +595,8 @@ int check_loss(const char* name, int dtype, const void* hidden, int hidden_dtype
     if (!weight || (rows > 0 && (!hidden || !loss))) return fail(PCD_INVALID_VALUE, "%s: null pointer", name);
     if (rows < 0 || dim < 1 || vocab < 1 || rows > (1 << 24) || dim > (1 << 20) || vocab > (1 << 24))
         return fail(PCD_INVALID_VALUE, "%s: bad shape: %d rows, dimension %d, vocabulary %d", name, rows, dim, vocab);
+    if ((long long)rows * vocab > kMostLogits)
+        return fail(PCD_INVALID_VALUE, "%s: %d rows of a vocabulary of %d are more than 2^39 logits", name, rows, vocab);
     for (long long* ld : {ldh, ldw, ld_dh, ld_dw}) {
         if (*ld == 0) *ld = dim;
         if (*ld < dim || *ld > (1 << 30))

@@ -102,3 +102,10 @@ def test_tensor_forms_check_shapes_and_types():
     for call in bad:
         with pytest.raises(ArgumentException):
             call()
+
+
+def test_more_logits_than_are_counted_are_refused():
+    for rows, vocab in ((2 ** 24, 2 ** 15 + 1), (2 ** 15 + 1, 2 ** 24)):
+        assert "2^39" in refused(TokenOps.cross_entropy_device, **{**LOSS, "labels": P, "rows": rows, "vocab": vocab})
+        assert "2^39" in refused(TokenOps.distill_device, **{**LOSS, "teacher_ids": P, "teacher_logits": P, "top": 4,
+                                                             "rows": rows, "vocab": vocab})
