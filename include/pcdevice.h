@@ -117,7 +117,9 @@ int pcd_free_async(void* ptr, void* stream);
  * (CudaAllocator.cs:63-84). */
 int pcd_host_alloc(void** ptr, size_t bytes);
 int pcd_host_free(void* ptr);
-/* Releases every cached block of both pools (CudaAllocator.TrimPools). */
+/* Releases every cached block of both pools (CudaAllocator.TrimPools), and the
+ * scratch of GEMMs and token operators recorded into graphs (see the token
+ * operators): not while such a graph is still to be replayed. */
 int pcd_trim_pools(void);
 /* cudaMemcpy / cudaMemcpyAsync / cudaMemsetAsync, Interop/Cuda.cs:37-39 */
 int pcd_memcpy(void* dst, const void* src, size_t bytes, int kind);
@@ -190,7 +192,13 @@ int pcd_gemm_f16_batched(const uint16_t* dA, const uint16_t* dB, float* dC, int 
  * given they are the same or one of them is PCD_F32.  A loss takes up to 2^24
  * rows, ids and 2^39 logits, and a dim of up to 2^20.  Results do not depend on
  * the launch's timing: the same inputs give the same bits.  Scratch comes from
- * the library's pool.  Asynchronous on `stream`. */
+ * the library's pool.  Asynchronous on `stream`.
+ *
+ * A call may be recorded into a HIP graph, with no call before it.  Its scratch
+ * is then memory of the recording's own, which only the same recording's calls
+ * on the same stream share and only pcd_trim_pools gives back: a graph may be
+ * replayed on any stream, beside other graphs and eager calls, but not beside
+ * itself. */
 
 /* out[i] = scale * table[tokens[i]], i < count, table [vocab x dim].  A token
  * below 0 is padding and gives a row of zeros; one of vocab or more gives a row

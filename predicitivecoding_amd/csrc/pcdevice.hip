@@ -20,6 +20,7 @@
 #include <mutex>
 #include <new>
 #include <string>
+#include <tuple>
 #include <unordered_map>
 #include <vector>
 
@@ -114,6 +115,16 @@ struct Pool {
     std::unordered_map<void*, bool> synchronous;          // blocks from the hipMalloc fallback (freed with hipFree)
     std::map<int, std::vector<void*>> host_free;          // bucket -> pinned blocks
     std::unordered_map<void*, int> host_live;
+    // Scratch of recorded calls (see scratch_alloc): free blocks by size of each
+    // (device, recording, stream), and whose a block in use is.
+    struct RecKey {
+        int dev;
+        unsigned long long id;
+        void* stream;
+        bool operator<(const RecKey& o) const { return std::tie(dev, id, stream) < std::tie(o.dev, o.id, o.stream); }
+    };
+    std::map<RecKey, std::multimap<size_t, void*>> recorded;
+    std::unordered_map<void*, std::pair<RecKey, size_t>> recorded_live;
     static constexpr size_t kMaxCached = 32;
 };
 Pool& pool() {
@@ -188,6 +199,75 @@ int pool_free(void* ptr, hipStream_t stream) {
     }
     HIP_TRY(hipFreeAsync(ptr, stream));
     return PCD_SUCCESS;
+}
+
+// Scratch of a call.  An eager call's is a block of the pool, which is the
+// stream's again as soon as the call has queued its work.  A call recorded into a
+// graph runs again whenever the graph does, on any stream and beside any eager
+// call, so its scratch is the recording's own: a block taken while a stream
+// records serves that recording's other calls on the same stream, in its order,
+// and nothing else, until pcd_trim_pools (the library does not learn when a graph
+// goes).  It comes from hipMalloc: hipMallocAsync would be recorded itself, and
+// back its memory only while the graph holds it.  Relaxed mode lets this thread
+// allocate while streams record.
+int recording_of(hipStream_t stream, unsigned long long* id) {
+    *id = 0;
+    if (stream == nullptr) return PCD_SUCCESS;   // the legacy stream cannot record
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    hipGraph_t graph = nullptr;
+    unsigned long long at = 0;
+    HIP_TRY(hipStreamGetCaptureInfo_v2(stream, &status, &at, &graph, nullptr, nullptr));
+    if (status != hipStreamCaptureStatusNone) *id = at;
+    return PCD_SUCCESS;
+}
+
+int scratch_alloc(void** out, size_t bytes, hipStream_t stream) {
+    unsigned long long id = 0;
+    if (int st = recording_of(stream, &id)) return st;
+    if (id == 0 || bytes == 0) return pool_alloc(out, bytes, stream);
+    *out = nullptr;
+    Pool::RecKey key{0, id, (void*)stream};
+    HIP_TRY(hipGetDevice(&key.dev));
+    Pool& P = pool();
+    {
+        std::lock_guard<std::mutex> g(P.mu);
+        auto& blocks = P.recorded[key];
+        auto it = blocks.lower_bound(bytes);
+        if (it != blocks.end() && it->first / 2 <= bytes) {
+            *out = it->second;
+            P.recorded_live[*out] = {key, it->first};
+            blocks.erase(it);
+            return PCD_SUCCESS;
+        }
+    }
+    bytes = round_up(bytes, 4096);
+    void* p = nullptr;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    HIP_TRY(hipThreadExchangeStreamCaptureMode(&mode));
+    const hipError_t e = hipMalloc(&p, bytes);
+    HIP_TRY(hipThreadExchangeStreamCaptureMode(&mode));
+    if (e != hipSuccess) {
+        (void)hipGetLastError();   // a caller that can do without the block goes on to its launches
+        return from_hip(e, "scratch of a recorded call");
+    }
+    std::lock_guard<std::mutex> g(P.mu);
+    P.recorded_live[p] = {key, bytes};
+    *out = p;
+    return PCD_SUCCESS;
+}
+
+int scratch_free(void* ptr, hipStream_t stream) {
+    Pool& P = pool();
+    {
+        std::lock_guard<std::mutex> g(P.mu);
+        auto it = P.recorded_live.find(ptr);
+        if (it != P.recorded_live.end()) {
+            P.recorded[it->second.first].emplace(it->second.second, ptr);
+            P.recorded_live.erase(it);
+            return PCD_SUCCESS;
+        }
+    }
+    return pool_free(ptr, stream);
 }
 
 // ------------------------------------------------------------------ launch
@@ -1493,6 +1573,9 @@ int pcd_trim_pools(void) {
             P.synchronous.erase(p);
         }
     P.free_blocks.clear();
+    for (auto& kv : P.recorded)
+        for (auto& block : kv.second) (void)hipFree(block.second);
+    P.recorded.clear();
     for (auto& kv : P.host_free)
         for (void* p : kv.second) (void)hipHostFree(p);
     P.host_free.clear();
@@ -1704,9 +1787,9 @@ static int gemm_common(int dtype, const void* dA, const void* dB, float* dC, int
     };
     int st = PCD_SUCCESS;
     if (!direct_a && !mk_a)
-        if (!(st = pool_alloc(&pa, (size_t)batch * m * kl * ob, s))) st = pack(dA, m, trans_a, pa);
+        if (!(st = scratch_alloc(&pa, (size_t)batch * m * kl * ob, s))) st = pack(dA, m, trans_a, pa);
     if (!st && !direct_b && !kn_b)
-        if (!(st = pool_alloc(&pb, (size_t)batch * n * kl * ob, s))) st = pack(dB, n, !trans_b, pb);
+        if (!(st = scratch_alloc(&pb, (size_t)batch * n * kl * ob, s))) st = pack(dB, n, !trans_b, pb);
     std::vector<ProblemSet> sets(1);
     std::memset(&sets[0], 0, sizeof(ProblemSet));
     sets[0].n = 1;
@@ -1735,7 +1818,7 @@ static int gemm_common(int dtype, const void* dA, const void* dB, float* dC, int
             if (cost(r) < cost(ks)) ks = r;
         const size_t part_bytes = (size_t)t128 * ks * 128 * 128 * 4, cnt_bytes = round_up((size_t)t128 * 4, 16);
         // without scratch for it the product is not split
-        if (ks > 1 && pool_alloc(&part, part_bytes + cnt_bytes, s) == PCD_SUCCESS) {
+        if (ks > 1 && scratch_alloc(&part, part_bytes + cnt_bytes, s) == PCD_SUCCESS) {
             p.part = (float*)part;
             p.count = (int*)((char*)part + part_bytes);
             p.ksplit = ks;
@@ -1749,7 +1832,7 @@ static int gemm_common(int dtype, const void* dA, const void* dB, float* dC, int
         SplitScratch sc;
         sc.budget = cus;
         const size_t part_bytes = (size_t)sc.budget * 128 * 128 * 4, cnt_bytes = split_count_bytes((int)sc.budget);
-        if (!(st = pool_alloc(&part, part_bytes + cnt_bytes, s))) {
+        if (!(st = scratch_alloc(&part, part_bytes + cnt_bytes, s))) {
             sc.part = (float*)part;
             sc.count = (int*)((char*)part + part_bytes);
             assign_split(cus, 1, dtype, tile, sc, sets, tile.m == 32 ? kSplitMinStagesKsw : kSplitMinStages);
@@ -1778,7 +1861,7 @@ static int gemm_common(int dtype, const void* dA, const void* dB, float* dC, int
     }
     for (void* q : {pa, pb, part})
         if (q) {
-            const int st2 = pool_free(q, s);
+            const int st2 = scratch_free(q, s);
             if (!st) st = st2;
         }
     return st;

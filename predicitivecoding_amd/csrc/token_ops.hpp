@@ -320,7 +320,7 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
     const size_t part_bytes = (size_t)c.cus * 128 * 128 * 4, count_bytes = split_count_bytes(c.cus);
     const size_t o_split = m.add(part_bytes + count_bytes);
     void* block = nullptr;
-    if (int st = pool_alloc(&block, m.size, s)) return st;
+    if (int st = scratch_alloc(&block, m.size, s)) return st;
     m.base = (char*)block;
 
     auto run = [&]() -> int {
@@ -578,7 +578,7 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
         return PCD_SUCCESS;
     };
     const int st = run();
-    const int st2 = pool_free(block, s);
+    const int st2 = scratch_free(block, s);
     return st ? st : st2;
 }
 
@@ -710,7 +710,7 @@ int pcd_token_embed_grad(int dtype, void* d_table, long long ld_table, const int
         const size_t o_counts = small ? 0 : m.add((size_t)tiles * 256 * 4), o_totals = small ? 0 : m.add(256 * 4);
         const size_t o_parts = windows ? m.add((size_t)2 * windows * pitch * 4) : 0;
         void* block = nullptr;
-        if (int st = pool_alloc(&block, m.size, s)) return st;
+        if (int st = scratch_alloc(&block, m.size, s)) return st;
         m.base = (char*)block;
         auto run = [&]() -> int {
             const int *keys = nullptr, *pos = nullptr;
@@ -763,7 +763,7 @@ int pcd_token_embed_grad(int dtype, void* d_table, long long ld_table, const int
             });
         };
         const int st = run();
-        const int st2 = pool_free(block, s);
+        const int st2 = scratch_free(block, s);
         return st ? st : st2;
     });
 }
