@@ -234,8 +234,8 @@ int pcd_token_keep_logits(size_t bytes);
  *   d_hidden [rows x dim] in hidden's type, d_weight [vocab x dim] in weight's.
  * row_weight null: 1.  A row with a negative label or weight 0 is left out: its
  * loss and its row of d_hidden are 0 and it adds nothing to d_weight, whatever
- * its hidden state holds.  A label of vocab or more makes the row's loss NaN
- * and leaves it out of the gradients.  Hidden states have weight's type, or
+ * its hidden state holds.  A label of vocab or more makes the loss NaN of a row
+ * whose weight is not 0 and leaves it out of the gradients.  Hidden states have weight's type, or
  * are fp32 beside a 16-bit weight (rounded to its type for the products, as
  * pcd_gemm_f16's operands; d_hidden is then fp32).  With gradients of 16-bit
  * types and more than 64 rows the loss's gradient by the logits is rounded to
@@ -255,8 +255,8 @@ int pcd_token_xent(int dtype, const void* hidden, int hidden_dtype, long long ld
  * A slot with a negative id, or a logit of minus infinity, is not there,
  * whatever else it holds; slots of equal ids are one of their summed
  * probability.  A row without a slot is left out as above; an id of vocab or
- * more makes the row's loss NaN and leaves it out of the gradients.
- * Everything else as pcd_token_xent. */
+ * more makes the loss NaN of a row whose weight is not 0 and leaves it out of
+ * the gradients.  Everything else as pcd_token_xent. */
 int pcd_token_distill(int dtype, const void* hidden, int hidden_dtype, long long ld_hidden, const void* weight,
                       long long ld_weight, const int* teacher_ids, const void* teacher_logits, int teacher_dtype, int top,
                       const float* row_weight, int rows, int dim, int vocab, float scale, float temperature, float* loss,

@@ -162,7 +162,7 @@ struct RowArgs {
     TokCtl* ctl;
     int* map;                  // caller's row of each live row
     int* rank;                 // live row of each caller's row, -1 where it is left out
-    float* loss;               // rows left out get 0 (a mark past the limit: NaN)
+    float* loss;               // rows left out get 0 (a mark past the limit and a weight: NaN)
     int stack;                 // few rows: the second copy of each lies this many rows on (0: there is none)
     RangeArgs dh;
     u32x4* clear;              // counters of the products' split K, cleared on the way (nullable)
@@ -177,6 +177,11 @@ __device__ __forceinline__ bool row_live(const RowArgs& a, int i) {
 }
 __device__ __forceinline__ float row_size(const RowArgs& a, int i) {
     return a.row_weight != nullptr ? fabsf(gld(a.row_weight + i)) : 1.f;
+}
+
+__device__ __forceinline__ float row_left_out(const RowArgs& a, int i) {
+    const bool past = gld(a.marks + i) >= a.limit && (a.row_weight == nullptr || gld(a.row_weight + i) != 0.f);
+    return past ? __builtin_nanf("") : 0.f;
 }
 
 // Gradients by the logits are held as multiples of the largest weight, so that
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const RowArgs a, const
     if (i < a.rows && lane == 0 && blockIdx.y == 0) {
         a.rank[i] = mine_live ? rank : -1;
         if (mine_live) a.map[rank] = i;
-        else a.loss[i] = gld(a.marks + i) >= a.limit ? __builtin_nanf("") : 0.f;
+        else a.loss[i] = row_left_out(a, i);
     }
     if (mine_live) {
 #pragma unroll
@@ -562,7 +567,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const RowArgs a, const To
         const int r = __popcll(lives & ((1ull << lane) - 1));
         a.rank[lane] = mine ? r : -1;
         if (mine) a.map[r] = lane;
-        else a.loss[lane] = gld(a.marks + lane) >= a.limit ? __builtin_nanf("") : 0.f;
+        else a.loss[lane] = row_left_out(a, lane);
     }
     int orig[NR];
     uint64_t rest = lives;
