@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(256) teacher_kernel(const int* __restrict__ id
     int past = 0;
     for (int j = threadIdx.x; j < top; j += 256) {
         int v = gld(ids + row * top + j);
-        const float x = OpTraits<TT>::load(logits, row * top + j) * inv_t;
+        const float x = OpTraits<TT>::load(logits, row * top + j);
         past |= v >= vocab;
         const bool there = v >= 0 && v < vocab && x != -__builtin_inff();
         raw_id[j] = there ? v : none;
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(256) teacher_kernel(const int* __restrict__ id
         const int v = raw_id[j];
         for (int k = 0; k < top; ++k) place += raw_id[k] < v || (raw_id[k] == v && k < j);
         id[place] = v;
-        t[place] = v == none ? 0.f : expf(raw_t[j] - m);
+        t[place] = v == none ? 0.f : expf((raw_t[j] - m) * inv_t);   // (a logit over T may overflow, this only to 0)
     }
     __syncthreads();
     float sum = 0.f;
