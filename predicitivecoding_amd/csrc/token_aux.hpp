@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(256) teacher_kernel(const int* __restrict__ id
     for (int j = threadIdx.x; j < top; j += 256) {
         int v = gld(ids + row * top + j);
         const float x = OpTraits<TT>::load(logits, row * top + j);
-        past |= v >= vocab;
+        past |= v >= vocab && x != -__builtin_inff();
         const bool there = v >= 0 && v < vocab && x != -__builtin_inff();
         raw_id[j] = there ? v : none;
         raw_t[j] = there ? x : -__builtin_inff();
