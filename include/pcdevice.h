@@ -241,7 +241,8 @@ int pcd_token_keep_logits(size_t bytes);
  * types and more than 64 rows the loss's gradient by the logits is rounded to
  * that type, once, before its products (of fewer rows it goes in two parts, of up
  * to 4 in fp32).  A weight with a row that is not finite gives losses
- * that are not finite.  rows = 0 writes no loss and a d_weight of zeros. */
+ * that are not finite.  rows = 0 writes no loss and a d_weight of zeros.
+ * scale log2(e) must be finite in fp32. */
 int pcd_token_xent(int dtype, const void* hidden, int hidden_dtype, long long ld_hidden, const void* weight,
                    long long ld_weight, const int* labels, const float* row_weight, int rows, int dim, int vocab,
                    float scale, float* loss, void* d_hidden, long long ld_dhidden, void* d_weight, long long ld_dweight,
@@ -256,7 +257,9 @@ int pcd_token_xent(int dtype, const void* hidden, int hidden_dtype, long long ld
  * whatever else it holds; slots of equal ids are one of their summed
  * probability.  A row without a slot is left out as above; an id of vocab or
  * more makes the loss NaN of a row whose weight is not 0 and leaves it out of
- * the gradients.  Everything else as pcd_token_xent. */
+ * the gradients.  scale log2(e) / temperature and scale temperature must be
+ * finite in fp32, temperature^2 a normal number.  Everything else as
+ * pcd_token_xent. */
 int pcd_token_distill(int dtype, const void* hidden, int hidden_dtype, long long ld_hidden, const void* weight,
                       long long ld_weight, const int* teacher_ids, const void* teacher_logits, int teacher_dtype, int top,
                       const float* row_weight, int rows, int dim, int vocab, float scale, float temperature, float* loss,

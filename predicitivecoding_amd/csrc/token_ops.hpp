@@ -185,6 +185,8 @@ constexpr int kTokStackRows = 64;
 constexpr int kSlimLeast = 384;
 constexpr size_t kSlimBytes = (size_t)112 << 20;
 
+constexpr float kLog2E = 1.4426950408889634f;
+
 struct Teacher {
     const int* ids;
     const void* logits;
@@ -340,7 +342,7 @@ int token_loss(int dtype, const void* hidden, int hidden_dtype, long long ldh, c
         k.taken = m.at<float>(o_taken);
         k.lse2 = m.at<float>(o_lse);
         const float inv_t = teacher ? 1.f / teacher->temperature : 1.f;
-        k.scale2 = scale * inv_t * 1.4426950408889634f;
+        k.scale2 = scale * inv_t * kLog2E;
         k.tail_stage = 0x7FFFFFFF;
         k.loss = loss;
         k.factor = 1.f;
@@ -587,7 +589,7 @@ constexpr long long kMostLogits = 1ll << 39;
 
 // The checks both losses make.
 int check_loss(const char* name, int dtype, const void* hidden, int hidden_dtype, long long* ldh, const void* weight,
-               long long* ldw, int rows, int dim, int vocab, float scale, const float* loss, long long* ld_dh,
+               long long* ldw, int rows, int dim, int vocab, float scale, float temperature, const float* loss, long long* ld_dh,
                long long* ld_dw) {
     if (!types_fit(dtype, hidden_dtype) || (dtype == PCD_F32 && hidden_dtype != PCD_F32))
         return fail(PCD_INVALID_VALUE, "%s: types %d and %d (hidden states have the weight's type or are fp32)", name, dtype,
@@ -602,7 +604,11 @@ int check_loss(const char* name, int dtype, const void* hidden, int hidden_dtype
         if (*ld < dim || *ld > (1 << 30))
             return fail(PCD_INVALID_VALUE, "%s: rows of %d elements are %lld apart", name, dim, *ld);
     }
-    if (!std::isfinite(scale)) return fail(PCD_INVALID_VALUE, "%s: the scale is not finite", name);
+    // the factors of the logits in base 2, of their gradients and of the losses
+    if (!std::isfinite(scale * (1.f / temperature) * kLog2E) || !std::isfinite(scale * temperature))
+        return fail(PCD_INVALID_VALUE, "%s: a scale of %g at a temperature of %g is not finite in fp32", name, scale, temperature);
+    if (!std::isnormal(temperature * temperature))
+        return fail(PCD_INVALID_VALUE, "%s: the square of a temperature of %g is not a normal fp32 number", name, temperature);
     return PCD_SUCCESS;
 }
 
@@ -612,7 +618,7 @@ int pcd_token_xent(int dtype, const void* hidden, int hidden_dtype, long long ld
                    long long ld_weight, const int* labels, const float* row_weight, int rows, int dim, int vocab, float scale,
                    float* loss, void* d_hidden, long long ld_dhidden, void* d_weight, long long ld_dweight, void* stream) {
     if (int st = check_loss("pcd_token_xent", dtype, hidden, hidden_dtype, &ld_hidden, weight, &ld_weight, rows, dim, vocab,
-                            scale, loss, &ld_dhidden, &ld_dweight))
+                            scale, 1.f, loss, &ld_dhidden, &ld_dweight))
         return st;
     if (rows > 0 && !labels) return fail(PCD_INVALID_VALUE, "pcd_token_xent: null labels");
     return guarded("pcd_token_xent", [&] {
@@ -625,15 +631,15 @@ int pcd_token_distill(int dtype, const void* hidden, int hidden_dtype, long long
                       long long ld_weight, const int* teacher_ids, const void* teacher_logits, int teacher_dtype, int top,
                       const float* row_weight, int rows, int dim, int vocab, float scale, float temperature, float* loss,
                       void* d_hidden, long long ld_dhidden, void* d_weight, long long ld_dweight, void* stream) {
+    if (!std::isfinite(temperature) || !(temperature > 0.f) || !std::isfinite(1.f / temperature))
+        return fail(PCD_INVALID_VALUE, "pcd_token_distill: the temperature is not a positive number with a finite inverse");
     if (int st = check_loss("pcd_token_distill", dtype, hidden, hidden_dtype, &ld_hidden, weight, &ld_weight, rows, dim,
-                            vocab, scale, loss, &ld_dhidden, &ld_dweight))
+                            vocab, scale, temperature, loss, &ld_dhidden, &ld_dweight))
         return st;
     if (rows > 0 && (!teacher_ids || !teacher_logits)) return fail(PCD_INVALID_VALUE, "pcd_token_distill: null teacher");
     if (!known_type(teacher_dtype)) return fail(PCD_INVALID_VALUE, "pcd_token_distill: unknown teacher type %d", teacher_dtype);
     if (top < 1 || top > kMaxTop)
         return fail(PCD_INVALID_VALUE, "pcd_token_distill: %d slots a row (1 to %d)", top, kMaxTop);
-    if (!std::isfinite(temperature) || !(temperature > 0.f) || !std::isfinite(1.f / temperature))
-        return fail(PCD_INVALID_VALUE, "pcd_token_distill: the temperature is not a positive number with a finite inverse");
     const Teacher t{teacher_ids, teacher_logits, teacher_dtype, top, temperature};
     return guarded("pcd_token_distill", [&] {
         return token_loss(dtype, hidden, hidden_dtype, ld_hidden, weight, ld_weight, nullptr, &t, row_weight, rows, dim,

@@ -109,3 +109,12 @@ def test_more_logits_than_are_counted_are_refused():
         assert "2^39" in refused(TokenOps.cross_entropy_device, **{**LOSS, "labels": P, "rows": rows, "vocab": vocab})
         assert "2^39" in refused(TokenOps.distill_device, **{**LOSS, "teacher_ids": P, "teacher_logits": P, "top": 4,
                                                              "rows": rows, "vocab": vocab})
+
+
+def test_factors_that_fp32_does_not_hold_are_refused():
+    ok = {**LOSS, "teacher_ids": P, "teacher_logits": P, "top": 4}
+    for bad in (dict(scale=3e38), dict(scale=-2.5e38)):   # times log2 e
+        refused(TokenOps.cross_entropy_device, **{**LOSS, "labels": P, **bad})
+    for bad in (dict(temperature=2e19), dict(temperature=1e-20), dict(scale=1e30, temperature=1e-9),
+                dict(scale=-1e30, temperature=1e9)):
+        refused(TokenOps.distill_device, **{**ok, **bad})
