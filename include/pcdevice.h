@@ -202,7 +202,7 @@ int pcd_gemm_f16_batched(const uint16_t* dA, const uint16_t* dB, float* dC, int 
 
 /* out[i] = scale * table[tokens[i]], i < count, table [vocab x dim].  A token
  * below 0 is padding and gives a row of zeros; one of vocab or more gives a row
- * of NaN. */
+ * of NaN.  dim is at most 2^30. */
 int pcd_token_embed(int dtype, const void* table, long long ld_table, const int* tokens, int count, int vocab, int dim,
                     float scale, void* out, int out_dtype, long long ld_out, void* stream);
 
@@ -210,7 +210,8 @@ int pcd_token_embed(int dtype, const void* table, long long ld_table, const int*
  * = v, zero in the rows that no token asked for; with `accumulate` the sum is
  * added to d_table instead, and rows that no token asked for are not touched
  * (a table shared with the output matrix adds to that one's gradient).  Tokens
- * outside [0, vocab) are left out.  Each token's positions are summed in their
+ * outside [0, vocab) are left out.  Up to 2^28 tokens, a vocab and a dim of up to
+ * 2^30.  Each token's positions are summed in their
  * order (sorted, no atomics on values). */
 int pcd_token_embed_grad(int dtype, void* d_table, long long ld_table, const int* tokens, int count, int vocab, int dim,
                          float scale, int accumulate, const void* d_out, int out_dtype, long long ld_out, void* stream);

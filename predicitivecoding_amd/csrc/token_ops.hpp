@@ -612,6 +612,9 @@ int check_loss(const char* name, int dtype, const void* hidden, int hidden_dtype
     return PCD_SUCCESS;
 }
 
+// Most elements of an embedding's row: units and a wave's columns past its end are still an int.
+constexpr int kMostDim = 1 << 30;
+
 }  // namespace
 
 int pcd_token_xent(int dtype, const void* hidden, int hidden_dtype, long long ld_hidden, const void* weight,
@@ -656,7 +659,7 @@ int pcd_token_embed(int dtype, const void* table, long long ld_table, const int*
                     float scale, void* out, int out_dtype, long long ld_out, void* stream) {
     if (!types_fit(dtype, out_dtype))
         return fail(PCD_INVALID_VALUE, "pcd_token_embed: types %d and %d", dtype, out_dtype);
-    if (count < 0 || vocab < 1 || dim < 1)
+    if (count < 0 || vocab < 1 || dim < 1 || dim > kMostDim)
         return fail(PCD_INVALID_VALUE, "pcd_token_embed: bad shape: %d tokens, vocabulary %d, dimension %d", count, vocab, dim);
     if (!table || (count > 0 && (!tokens || !out))) return fail(PCD_INVALID_VALUE, "pcd_token_embed: null pointer");
     if (ld_table == 0) ld_table = dim;
@@ -679,7 +682,7 @@ int pcd_token_embed_grad(int dtype, void* d_table, long long ld_table, const int
     hipStream_t s = (hipStream_t)stream;
     if (!types_fit(dtype, out_dtype))
         return fail(PCD_INVALID_VALUE, "pcd_token_embed_grad: types %d and %d", dtype, out_dtype);
-    if (count < 0 || count > (1 << 28) || vocab < 1 || vocab > (1 << 30) || dim < 1)
+    if (count < 0 || count > (1 << 28) || vocab < 1 || vocab > (1 << 30) || dim < 1 || dim > kMostDim)
         return fail(PCD_INVALID_VALUE, "pcd_token_embed_grad: bad shape: %d tokens, vocabulary %d, dimension %d", count, vocab,
                     dim);
     if (!d_table || (count > 0 && (!tokens || !d_out))) return fail(PCD_INVALID_VALUE, "pcd_token_embed_grad: null pointer");

@@ -118,3 +118,10 @@ def test_factors_that_fp32_does_not_hold_are_refused():
     for bad in (dict(temperature=2e19), dict(temperature=1e-20), dict(scale=1e30, temperature=1e-9),
                 dict(scale=-1e30, temperature=1e9)):
         refused(TokenOps.distill_device, **{**ok, **bad})
+
+
+def test_rows_longer_than_an_int_counts_units_of_are_refused():
+    # the last unit of a row, and a wave's last column, end past it
+    for dim in (2 ** 30 + 1, 2 ** 31 - 1):
+        refused(TokenOps.embed_device, "bf16", P, P, 1, 1, dim, P)
+        refused(TokenOps.embed_grad_device, "bf16", P, P, 1, 1, dim, P)
