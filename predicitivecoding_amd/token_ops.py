@@ -76,7 +76,7 @@ class TokenOps:
         """scale * table[tokens] as [tokens x dim], of the table's type or `out_dtype` (fp32 beside a 16-bit table: what
         a settling takes).  Tokens below 0 are padding: rows of zeros."""
         vocab, dim = _matrix(table, "table")
-        _ints(tokens, tokens.shape[:1], "tokens")
+        _ints(tokens, tokens.shape[:1] or (1,), "tokens")
         n = tokens.shape[0]
         if out is None:
             out = DeviceTensor((n, dim), out_dtype or table.dtype, stream)

@@ -125,3 +125,8 @@ def test_rows_longer_than_an_int_counts_units_of_are_refused():
     for dim in (2 ** 30 + 1, 2 ** 31 - 1):
         refused(TokenOps.embed_device, "bf16", P, P, 1, 1, dim, P)
         refused(TokenOps.embed_grad_device, "bf16", P, P, 1, 1, dim, P)
+
+
+def test_tokens_without_an_axis_are_refused():
+    with pytest.raises(ArgumentException):
+        TokenOps.embed(Fake((10, 8), np.float32), Fake((), np.int32))
