@@ -515,7 +515,8 @@ template <typename OP> __device__ __forceinline__ float dot_word(uint32_t a, uin
 // streams W.  A product of so few rows is W's read and nothing else; a wave takes
 // four of W's rows at a time, whole, 16 bytes a lane, against the hidden states
 // in LDS.  The 4 NR sums over its lanes halve as they go (each lane keeps half of
-// what it holds and gives the other half away: 4 NR + 1 exchanges for up to 24 NR),
+// what it holds and gives the other half away: 7, 10, 17 and 32 exchanges with 1,
+// 2, 4 and 8 rows, for 24 NR),
 // and a lane keeps the running sum of its own logits.  Every workgroup finds the
 // live ones of the few rows by itself.  All logits are kept, 4 bytes to a row of
 // W.  `nt`: W is larger than the caches, so its lines are not kept in them.

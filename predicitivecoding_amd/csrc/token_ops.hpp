@@ -179,9 +179,12 @@ constexpr int kTokStackRows = 64;
 
 // Few rows' DW takes slim_dw_kernel, whose workgroups want 512 columns, from
 // kSlimLeast of them on, but beside DH only from kSlimBytes of output on: below,
-// what one launch for both saves is more (us of a call with both gradients, slim
-// and not: 16 x 32000 x 2048 bf16 119 / 126, 40 x 50257 x 1024 126 / 122, 64 x 10000 x
-// 784 49 / 48; d_weight alone 77 / 86, 79 / 89, 32 / 35).
+// what one launch for both saves is more.  Calls with both gradients of 8 to 64 rows,
+// bf16, 512 to 4096 columns, on the tiles and slim: outputs of 128 to 384 MB 0.97 to
+// 1.13 (1.04 in the mean of up to 32 rows, 1.06 of more), 64 and 96 MB 0.93 to 1.06
+// (1.03 and 0.99), 16 and 32 MB 0.87 to 1.02 (0.99 and 0.91).  d_weight alone, us slim
+// and not: 16 x 32000 x 2048 bf16 77 / 86, 40 x 50257 x 1024 79 / 89, 64 x 10000 x 784
+// 32 / 35.
 constexpr int kSlimLeast = 384;
 constexpr size_t kSlimBytes = (size_t)112 << 20;
 
